@@ -696,8 +696,10 @@ cudaError_t launch_kv_attn(const KvAttention& a0, const KvCache& c, const KvBatc
   const int64_t from = tile_rows_from(c.dim, a.rows * a.group * c.heads);
   if (kv_prefill_takes(c.dim, bf16) && a.rows * a.group > from && (most > from || max_new == 0)) {
     a.rows_above = a.rows_upto = from;
+    // One sequence is the tile kernel's whatever rows q_start gives it, which may be fewer than the tensor has.
+    if (b.seqs == 1) a.rows_above = -1;
     cudaError_t e = launch_kv_prefill(a, c, b, ws, st);
-    if (e != cudaSuccess || b.seqs == 1) return e;  // one sequence: all the rows are its own
+    if (e != cudaSuccess || b.seqs == 1) return e;
   }
   switch (c.dim) {
     case 64: return bf16 ? kv::pick<64, false>(a, c, b, max_new, ws, st) : kv::pick<64, true>(a, c, b, max_new, ws, st);
