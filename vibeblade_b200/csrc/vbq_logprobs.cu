@@ -36,6 +36,7 @@ constexpr float kSlack = 8.0f;
 constexpr int kSliceThreads = 256;
 constexpr int kFew = 4;             // vectors a thread, up to which lanes look at their own
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = 1e30f;       // from here on x - r can leave fp32, or r be a type's lowest value
 constexpr int kUnroll = 2;         // vectors on their way a thread (4: 125 us against 114 over 525 MB)
 constexpr int kMaxSplits = 128, kMaxSplitRows = 512;
 
@@ -103,7 +104,8 @@ template <bool BF16> struct Row {
   }
 };
 
-// -inf as the type's lowest value (its weight is 0 either way, and 0 times it is 0); NaN stays
+// -inf as the type's lowest value; NaN stays.  Beside a larger reference the weight is 0 either way, and
+// 0 times it is 0; a slice that has nothing larger is summed again (kFar).
 __device__ __forceinline__ uint32_t floor2(uint32_t w) {
   const __nv_bfloat162 lo = __halves2bfloat162(__ushort_as_bfloat16(0xff7f), __ushort_as_bfloat16(0xff7f));
   const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&w), lo);
@@ -362,6 +364,29 @@ logprobs_kernel(const void* __restrict__ logits, int64_t stride, int64_t vocab, 
   s = sh.part[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) s = joined(s, sh.part[w]);
+  // A largest logit this far out, which the pass's shortcuts do not hold for: -inf, read there as the
+  // type's lowest value, would weigh as much as that, and x - r may be -inf.  Rows whose every token
+  // is masked come here, so the slice is summed once more, element by element.
+  if (fabsf(s.r) >= kFar && fabsf(s.r) < INFINITY) {
+    Sums t{s.r, 0.0f, 0.0f};
+    for (int e = x_row.e0 + tid; e < x_row.e1; e += kThreads) {
+      const float d = x_row.one(e) - s.r;
+      const float y = ex2(d * kLog2e);  // 0 for -inf, NaN for NaN
+      t.z += y;
+      if (y > 0.0f) t.b = fmaf(d, y, t.b);
+    }
+    __syncthreads();  // every thread has read the sums of before
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      t.z += __shfl_xor_sync(kFull, t.z, o);
+      t.b += __shfl_xor_sync(kFull, t.b, o);
+    }
+    if (lane == 0) sh.part[warp] = t;
+    __syncthreads();
+    s = sh.part[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) s.z += sh.part[w].z, s.b += sh.part[w].b;
+  }
 
   if (splits > 1) {
     float* mine = slices + (row * splits + blockIdx.x) * slice_words(top);
