@@ -1,0 +1,58 @@
+"""Attention over values and queries at the ends of their ranges, and over long caches.  Tolerances as
+in tests/test_kv_gpu.py."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import vibeblade_b200 as vb
+
+pytestmark = pytest.mark.gpu
+
+
+def _two_scores(cuda, dtype, new, dim, values):
+    """8 KV heads of 8 query heads over 40960 tokens, of which the first 128 score 0 and the others
+    7.8 log 2: (out, lse, the second score, codes, scales)."""
+    kv, group, page, L = 8, 8, 128, 40960
+    n = L // page
+    g = torch.Generator(device=cuda).manual_seed(dim)
+    codes = torch.zeros((n, 1, 2, kv, page, dim), dtype=torch.int8, device=cuda)
+    scales = torch.zeros((n, 1, 2, kv), device=cuda)
+    codes[1:, :, 0] = 127
+    scale = dim ** -0.5
+    ks = float(np.float32(7.8 * math.log(2) / (127 * dim * scale)))
+    scales[1:, :, 0] = ks
+    if values:
+        codes[:, :, 1] = torch.randint(-127, 128, codes[:, :, 1].shape, generator=g, dtype=torch.int8, device=cuda)
+        scales[:, :, 1] = 0.005 + 0.02 * torch.rand(scales[:, :, 1].shape, generator=g, device=cuda)
+    q = torch.ones(new, kv * group * dim, dtype=dtype, device=cuda)
+    tables = torch.arange(n, dtype=torch.int32, device=cuda)[None].contiguous()
+    out, lse = vb.kv_attention(q, codes, scales, tables, torch.tensor([L], dtype=torch.int32, device=cuda),
+                               torch.tensor([0, new], dtype=torch.int32, device=cuda), max_new=new, with_lse=True)
+    s = 127 * dim * ks * scale
+    seen = L - new + np.arange(new) + 1
+    ref_lse = np.log(page + (seen - page) * math.exp(s))
+    assert np.abs(lse.double().cpu().numpy() - ref_lse[:, None]).max() <= 2e-5 + 2.0 ** -22 * ref_lse.max()
+    return out, s, codes, scales
+
+
+@pytest.mark.parametrize("dtype,new", [(torch.bfloat16, 600), (torch.bfloat16, 1), (torch.float32, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_caches_of_equal_scores(cuda, dtype, new, dim):
+    """Tens of thousands of equal weights: their sum's roundings go one way."""
+    out, s, codes, scales = _two_scores(cuda, dtype, new, dim, True)
+    page, kv, L = 128, 8, 40960
+    v = (codes[:, 0, 1].double() * scales[:, 0, 1].double()[..., None, None]).permute(0, 2, 1, 3).reshape(L, kv, dim)
+    v[page:] *= math.exp(s)
+    seen = L - new + torch.arange(new, device=cuda)
+    z = page + (seen + 1 - page).double() * math.exp(s)
+    ref = v.cumsum(0)[seen] / z[:, None, None]
+    err = (out.double().view(new, kv, 8, dim) - ref[:, :, None]).abs()
+    vmax = 127 * float(scales.max())
+    if dtype == torch.float32:
+        assert err.max() <= 2e-5 * vmax
+    else:
+        assert (err <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref[:, :, None].abs()).all()

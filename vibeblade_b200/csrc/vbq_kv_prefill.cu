@@ -566,6 +566,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
             }
           }
         }
+        float of_run = 0.0f;  // added up by itself first: l takes a rounding a run, not one a block
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           uint32_t pk[16];
@@ -582,7 +583,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
               sum = __fadd2_rn(sum, v);
               pk[8 * x + y / 2] = h2(v.x, v.y);
             }
-            l = fmaf(sum.x + sum.y, p.iv, l);
+            of_run = fmaf(sum.x + sum.y, p.iv, of_run);
           }
           p_st16(ts + 16 * h, pk);
           if (h == 1) {  // the second product may begin on these
@@ -592,6 +593,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
             if (lane == 0) mbar_arrive(smem_u32(&bars.p_half[half]));
           }
         }
+        l += of_run;
         p_wait_st();
         p_fence_before();
         __syncwarp();
