@@ -56,3 +56,12 @@ def test_long_caches_of_equal_scores(cuda, dtype, new, dim):
         assert err.max() <= 2e-5 * vmax
     else:
         assert (err <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref[:, :, None].abs()).all()
+
+
+@pytest.mark.parametrize("dtype,new", [(torch.bfloat16, 600), (torch.bfloat16, 1), (torch.float32, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_caches_of_zero_values(cuda, dtype, new, dim):
+    """Blocks of zeros have the scale 0; the sum of exponentials over them stays in range when the later
+    scores lie 2^7.8 above the first ones', which a lazily moved reference lets pass."""
+    out = _two_scores(cuda, dtype, new, dim, False)[0]
+    assert (out == 0).all()

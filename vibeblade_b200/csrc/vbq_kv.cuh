@@ -29,6 +29,11 @@ __device__ __forceinline__ int64_t block_index(const KvCache& c, int page, int w
   return (((int64_t)page * c.layers + c.layer) * 2 + which) * c.heads + head;
 }
 
+// A value block's scale as the attention's weights take it.  They carry it, and the sum of exponentials
+// takes its reciprocal: a block of zeros, whose scale is 0 and any would do, gets one that leaves the
+// sum of 2^24 tokens' weights (2^15 at most) in fp32 and lies below every scale that matters.
+__device__ __forceinline__ float value_scale(float vs) { return vs == 0.0f ? 0x1p-60f : fmaxf(vs, 1e-30f); }
+
 // a / b of numbers that are not negative, by the short division where both are short.
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return ((a | b) >> 32) ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);

@@ -392,9 +392,8 @@ attn_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, int*
             mma16832(si[t][k], word(kr[0], w), word(kr[1], w), word(kr[0], w + 1), word(kr[1], w + 1),
                      sh_q[t][k][w >> 1][lane][0], sh_q[t][k][w >> 1][lane][1]);
         }
-      // vs = 2^e f.  A block of zeros has scale 0, and any scale will do for it (the floor is for
-      // that, and takes values below 1.3e-28 to at most that)
-      const uint32_t vb = __float_as_uint(fmaxf(vs, 1e-30f));
+      // vs = 2^e f, at least 1e-30 (values below 1.3e-28 are taken as up to that)
+      const uint32_t vb = __float_as_uint(value_scale(vs));
       const float vec = vs == -INFINITY ? -INFINITY : (float)((int)(vb >> 23) - 127);  // no page: no weight
       const float vfc = __uint_as_float((vb & 0x7fffffu) | 0x3f800000u);
       const float vdc = __uint_as_float((254u << 23) - (vb & 0x7f800000u));

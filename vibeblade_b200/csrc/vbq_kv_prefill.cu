@@ -880,7 +880,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
           const int page = tok < len ? page_of(c, b, s, tok >> c.page_log2) : -1;
           if (page >= 0) {
             const float* q = base + (int64_t)page * c.layers * 2 * c.heads;
-            const float v = fmaxf(__ldg(q + c.heads), 1e-30f);  // see vbq_kv_attn.cu
+            const float v = value_scale(__ldg(q + c.heads));
             p = {__ldg(q), log2f(v), __fdiv_rn(1.0f, v), 0.0f};
           }
           wait(bars.scale_empty[count % kScaleRing], ((count / kScaleRing) & 1) ^ 1);
