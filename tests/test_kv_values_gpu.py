@@ -8,7 +8,9 @@ import numpy as np
 import pytest
 import torch
 
+import kv_reference as R
 import vibeblade_b200 as vb
+from test_kv_gpu import DT, _check, _q
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +67,23 @@ def test_long_caches_of_zero_values(cuda, dtype, new, dim):
     scores lie 2^7.8 above the first ones', which a lazily moved reference lets pass."""
     out = _two_scores(cuda, dtype, new, dim, False)[0]
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("new", [1, 140])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_infinite_queries_give_nan_in_their_rows(cuda, dtype, new, value):
+    """Scores of +-inf or NaN have no softmax: the row is NaN, whatever the sign of the keys' codes."""
+    pool = R.Pool([260], 32, 128, 2, seed=8)
+    pool.codes[:, :, 0, :, :, 3] = -5  # one sign for every key
+    q, q64 = _q(new, 4 * 128, 1, dtype, cuda)
+    q[0, 3] = value
+    q64[0, :128] = 0
+    codes, scales, tables, ln = pool.on(cuda)
+    out, lse = vb.kv_attention(q, codes, scales, tables, ln, torch.tensor([0, new], dtype=torch.int32, device=cuda),
+                               with_lse=True, max_new=new)
+    assert torch.isnan(out[0, :128]).all() and torch.isnan(lse[0, 0])
+    ref, ref_lse = R.attention(pool, q64, [new], 4)
+    out[0, :128] = torch.from_numpy(ref[0, 0]).to(out)
+    lse[0, 0] = float(ref_lse[0, 0])
+    _check(out, lse, ref, ref_lse, 127 * float(pool.scales.max()), dtype)

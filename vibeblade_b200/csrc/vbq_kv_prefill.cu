@@ -492,8 +492,9 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const uint32_t v[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
-          // (a negative scale negates the row: score factors are not negative)
-          const float up = copysignf(__uint_as_float((uint32_t)(127 + shift(top[e])) << 23), a.scale);
+          // (a negative scale negates the row: score factors are not negative; an infinity or NaN in the
+          // row makes all of it NaN, as scores of -inf alone would pass for masked ones)
+          const float up = top[e] >= 0x7f800000u ? NAN : copysignf(__uint_as_float((uint32_t)(127 + shift(top[e])) << 23), a.scale);
           uint32_t h[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) h[k] = h2(bf_lo(v[k]) * up, bf_hi(v[k]) * up);
