@@ -76,7 +76,8 @@ int vbq_kv_attention_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t di
  * h / (heads / kv_heads).  q and out are [rows, heads * dim] of `dtype`, rows q_stride and
  * out_stride elements apart, 16-byte aligned with row strides of whole 16 bytes.  lse (fp32
  * [rows, heads], may be NULL) receives the natural log of the row's sum of exponentials.  A
- * row that sees no token gets zeros and -inf.
+ * row that sees no token, or that no sequence has (before q_start[0], from q_start[seqs] on), gets
+ * zeros and -inf.
  *
  * Codes are multiplied exactly and sums are fp32.  Queries enter to 2^-22 of their row's largest
  * value (bf16 prompts of dim 64 or 128: 11 bits of each, so all that bf16 has); softmax weights

@@ -35,3 +35,18 @@ def test_one_sequence_of_fewer_tokens_than_rows(cuda, dim, heads, kv_heads, rows
     out, lse, ref, ref_lse, vmax = _longer(cuda, [140 + new], [new], rows, heads, kv_heads, dim, torch.bfloat16,
                                            {"none": 0, "rows": rows, "right": new}[hint], seed=new)
     _check(out[:new].contiguous(), lse[:new], ref, ref_lse, vmax, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,new,lead,rows", [
+    ([90, 5], [2, 1], 0, 9), ([90, 5], [2, 1], 3, 6), ([300, 90], [150, 40], 2, 260), ([300], [150], 0, 400),
+    ([300], [0], 0, 200), ([40, 0], [0, 0], 0, 7), ([333, 50, 20], [1, 140, 1], 5, 147), ([30] * 40, [1] * 40, 1, 64),
+])
+def test_rows_of_no_sequence_see_nothing(cuda, dtype, dim, lens, new, lead, rows):
+    out, lse, ref, ref_lse, vmax = _longer(cuda, lens, new, rows, 8, 2, dim, dtype, 0, lead=lead, seed=rows)
+    n = sum(new)
+    if n:
+        _check(out[lead:lead + n].contiguous(), lse[lead:lead + n], ref, ref_lse, vmax, dtype)
+    for part in (slice(0, lead), slice(lead + n, rows)):
+        assert (out[part] == 0).all() and torch.isneginf(lse[part]).all()

@@ -115,6 +115,21 @@ cudaError_t launch_behind(void (*kern)(P...), dim3 grid, unsigned threads, size_
   return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 
+// Rows of the call that no sequence has, before q_start's first and from its last on, see no token: zeros
+// and -inf.  The grid's CTAs share the rows; there mostly are none.
+template <bool F32>
+__device__ __forceinline__ void blank_rows(const KvAttention& a, const KvCache& c, const KvBatch& b) {
+  const int from = __ldg(b.q_start), to = __ldg(b.q_start + b.seqs);
+  const int heads = c.heads * a.group, width = heads * (c.dim * (F32 ? 4 : 2) / 16);  // 16-byte pieces of a row
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (row >= from && row < to) continue;
+    uint4* out = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + row * a.out_stride * (F32 ? 4 : 2));
+    for (int x = threadIdx.x; x < width; x += blockDim.x) out[x] = make_uint4(0, 0, 0, 0);
+    if (a.lse)
+      for (int x = threadIdx.x; x < heads; x += blockDim.x) a.lse[row * heads + x] = -INFINITY;
+  }
+}
+
 constexpr float kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -163,7 +163,7 @@ attn_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, int*
   auto least = [&]() {
     return (int64_t)max(kMinChunks, (int)sqrtf(0.25f * (float)(int)__reduce_max_sync(kFull, (unsigned)longest)));
   };
-  int64_t total, per, u_begin;
+  int64_t total, per, u_begin;  // past `total` a CTA has no unit, and its loop no turn
   Unit unit;
   if (b.seqs <= 32) {  // one look at the sequences for both their sum and this CTA's place
     const int64_t mine = lane < b.seqs ? units(lane) : 0;
@@ -171,20 +171,12 @@ attn_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, int*
     total = __shfl_sync(kFull, end, 31);
     per = max(quotient(total + gridDim.x - 1, gridDim.x), least());
     u_begin = blockIdx.x * per;
-    if (u_begin >= total) {
-      pdl_wait();  // see the end
-      return;
-    }
     const int at = __ffs(__ballot_sync(kFull, end > u_begin)) - 1;
     unit = {at, u_begin - __shfl_sync(kFull, end - mine, at)};
   } else {
     total = count_units(b.seqs, lane, units);
     per = max(quotient(total + gridDim.x - 1, gridDim.x), least());
     u_begin = blockIdx.x * per;
-    if (u_begin >= total) {
-      pdl_wait();  // see the end
-      return;
-    }
     unit = find_unit(u_begin, b.seqs, lane, units);
   }
   const int64_t u_end = min(total, u_begin + per);
@@ -631,6 +623,7 @@ attn_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, int*
     unit.at += ch1 - ch0;
     if (unit.at == (int64_t)v.chunks * v.tiles * c.heads) unit = {s + 1, 0};
   }
+  if (__ldg(b.q_start) > 0 || __ldg(b.q_start + b.seqs) < a.rows) blank_rows<F32>(a, c, b);
   // Started under the tile kernel, this one needs nothing of it; but the call has ended only when both have.
   pdl_wait();
 }

@@ -382,6 +382,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
   }
   // the kernel for the sequences of few rows may use the SMs that this one leaves free
   if (b.seqs > 1) pdl_release();
+  else if (__ldg(b.q_start) > 0 || __ldg(b.q_start + 1) < a.rows) blank_rows<false>(a, c, b);
   // the runs of every sequence, a warp a sequence (by the schedule's warp alone, one after the other,
   // 45 sequences took 60 us)
   {

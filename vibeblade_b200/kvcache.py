@@ -80,8 +80,8 @@ def kv_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tab
     sequence's n new tokens sees the tokens up to its own, the last ``window`` of them if that
     is not 0.  ``scale`` defaults to dim ** -0.5.  ``max_new``: the most new tokens a sequence
     has, where known (it selects the kernel).  Returns out [rows, heads * dim], with
-    ``with_lse`` also the fp32 [rows, heads] log-sum-exp.  A row that sees nothing gives
-    zeros and -inf."""
+    ``with_lse`` also the fp32 [rows, heads] log-sum-exp.  A row that sees nothing, or
+    that no sequence has (before q_start's first and from its last on), gives zeros and -inf."""
     return (_F or _load()).attention(q, codes, scales, tables, lens, q_start, layer, scale, window, max_new, out,
                                      bool(with_lse))
 
