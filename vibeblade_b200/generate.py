@@ -49,12 +49,13 @@ class Decoder:
         self.head_type = F.parse_type(t)
         first = layers[0]
         self.dev, self.cfg, self.page = first.dev, first.cfg, page
-        self.max_pages = -(-max_tokens // page)
+        self.max_tokens, self.max_pages = max_tokens, -(-max_tokens // page)
         dim = self.cfg.head_dim
         self.codes, self.scales = kv_pool(pages, len(layers), first.kv_heads, page, dim, device=self.dev)
-        # build_rope_cache (vibeblade/transformer.py:102-112), float32 throughout
+        # build_rope_cache (vibeblade/transformer.py:102-112), float32 throughout; every position a row's
+        # pages can hold
         inv = 1.0 / (rope_theta ** (torch.arange(0, dim, 2, dtype=torch.float32) / dim))
-        angle = torch.outer(torch.arange(max_tokens, dtype=torch.float32), inv)
+        angle = torch.outer(torch.arange(self.max_pages * page, dtype=torch.float32), inv)
         self.cos, self.sin = angle.cos().to(self.dev), angle.sin().to(self.dev)
 
     def rows(self, n: int) -> Rows:
@@ -72,13 +73,15 @@ class Decoder:
 
     def forward(self, rows: Rows, tokens: torch.Tensor, new: list[int]) -> tuple[Rows, torch.Tensor]:
         """Append ``new[r]`` tokens to each row (``tokens`` [sum(new)], row after row) and run the
-        blocks on them.  Returns the rows and the last block's output [sum(new), hidden]."""
+        blocks on them.  Returns the rows and the last block's output [sum(new), hidden].  Tokens past
+        a row's pages count in ``missing`` and are not stored."""
         n = torch.tensor(new, dtype=torch.int32, device=self.dev)
         q_start = torch.zeros(len(new) + 1, dtype=torch.int32, device=self.dev)
         torch.cumsum(n, 0, out=q_start[1:])
         refs, tables, lens, missing = kv_reserve(rows.refs, rows.tables, rows.lens, n, self.page)
         row = torch.repeat_interleave(torch.arange(len(new), device=self.dev), n, output_size=sum(new))
         at = rows.lens.long()[row] + torch.arange(sum(new), device=self.dev) - q_start.long()[row]
+        at = at.clamp(max=self.cos.shape[0] - 1)  # past the row's pages there is no position
         x = self.embedding[tokens]
         prefill = x.shape[0] > DECODE_MAX_TOKENS
         for i, layer in enumerate(self.layers):
@@ -100,6 +103,7 @@ class Decoder:
     def score(self, prompts: list[list[int]]) -> list[torch.Tensor]:
         """Log probability of each prompt's tokens after its first, given those before."""
         new = [len(p) for p in prompts]
+        self._fits(max(new, default=0))
         tokens = torch.tensor([t for p in prompts for t in p], device=self.dev)
         rows, x = self.forward(self.rows(len(prompts)), tokens, new)
         self._have(rows)
@@ -112,6 +116,7 @@ class Decoder:
         """The ``beams`` best continuations found of ``steps`` tokens: (tokens [beams, steps], their
         log probabilities [beams]), best first.  Up to 32 beams."""
         dev = self.dev
+        self._fits(len(prompt) + max(steps - 1, 0))  # the last tokens are not run
         rows, x = self.forward(self.rows(1), torch.tensor(prompt, device=dev), [len(prompt)])
         logits = self.logits(x[-1:])
         total = torch.zeros(1, device=dev)
@@ -129,6 +134,10 @@ class Decoder:
             logits = self.logits(x)
         self._have(rows)
         return out, total
+
+    def _fits(self, tokens: int) -> None:
+        if tokens > self.max_tokens:
+            raise RuntimeError(f"Decoder: a row of {tokens} tokens, max_tokens is {self.max_tokens}")
 
     def _have(self, rows: Rows) -> None:
         short = int(rows.missing.item())
