@@ -66,3 +66,31 @@ def test_positions_stay_in_the_table(monkeypatch, length, new):
     rows.lens = lens
     after, x = d.forward(rows, torch.zeros(new, dtype=torch.long), [new])
     assert x.shape == (new, HIDDEN) and after.lens.item() == length + new
+
+
+@pytest.mark.parametrize("token", [VOCAB, -1, 1 << 40])
+def test_tokens_outside_the_vocabulary(no_launch, token):
+    d = decoder()
+    for call in (lambda: d.score([[1, 2], [3, token]]), lambda: d.beam_search([token, 1], 2, 3)):
+        with pytest.raises(RuntimeError, match="vocabulary"):
+            call()
+
+
+def test_searches_that_cannot_be(no_launch):
+    d = decoder()
+    for prompt, beams, steps, text in (([], 2, 3, "empty"), ([1], 0, 3, "beams"), ([1], 33, 3, "beams")):
+        with pytest.raises(RuntimeError, match=text):
+            d.beam_search(prompt, beams, steps)
+    with pytest.raises(RuntimeError, match="beams"):
+        decoder(vocab=5).beam_search([1], 6, 3)  # the first step has five tokens to choose from
+
+
+def test_embedding_smaller_than_the_vocabulary():
+    with pytest.raises(RuntimeError, match="embedding"):
+        decoder(vocab=VOCAB, rows=VOCAB - 1)
+    decoder(vocab=VOCAB, rows=VOCAB + 14)  # padded rows are no harm
+
+
+def test_nothing_to_score(no_launch):
+    assert decoder().score([]) == []
+    assert [t.numel() for t in decoder().score([[], []])] == [0, 0]

@@ -46,6 +46,8 @@ class Decoder:
                  rope_theta: float = 10000.0):
         self.layers, self.embedding, self.final_norm = layers, embedding, final_norm
         self.head, t, self.vocab = lm_head
+        if embedding.shape[0] < self.vocab:  # a chosen token is looked up there
+            raise RuntimeError(f"Decoder: an embedding of {embedding.shape[0]} rows for a vocabulary of {self.vocab}")
         self.head_type = F.parse_type(t)
         first = layers[0]
         self.dev, self.cfg, self.page = first.dev, first.cfg, page
@@ -104,6 +106,9 @@ class Decoder:
         """Log probability of each prompt's tokens after its first, given those before."""
         new = [len(p) for p in prompts]
         self._fits(max(new, default=0))
+        self._known(t for p in prompts for t in p)
+        if sum(new) == 0:
+            return [torch.empty(0, device=self.dev) for _ in prompts]
         tokens = torch.tensor([t for p in prompts for t in p], device=self.dev)
         rows, x = self.forward(self.rows(len(prompts)), tokens, new)
         self._have(rows)
@@ -114,15 +119,20 @@ class Decoder:
 
     def beam_search(self, prompt: list[int], beams: int, steps: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The ``beams`` best continuations found of ``steps`` tokens: (tokens [beams, steps], their
-        log probabilities [beams]), best first.  Up to 32 beams."""
+        log probabilities [beams]), best first.  Up to 32 beams, and as many as the vocabulary has."""
         dev = self.dev
+        if not 1 <= beams <= min(32, self.vocab):
+            raise RuntimeError(f"Decoder: beams must be in 1..{min(32, self.vocab)}, got {beams}")
+        if not prompt:
+            raise RuntimeError("Decoder: the prompt is empty")
+        self._known(prompt)
         self._fits(len(prompt) + max(steps - 1, 0))  # the last tokens are not run
         rows, x = self.forward(self.rows(1), torch.tensor(prompt, device=dev), [len(prompt)])
         logits = self.logits(x[-1:])
         total = torch.zeros(1, device=dev)
         out = torch.empty((1, 0), dtype=torch.int32, device=dev)
         for step in range(steps):
-            _, _, lp, tok = token_logprobs(logits, None, min(beams, self.vocab))
+            _, _, lp, tok = token_logprobs(logits, None, beams)
             best, at = torch.topk((total[:, None] + lp).view(-1), beams)
             parents = (at // lp.shape[1]).to(torch.int32)
             total, chosen = best, tok.view(-1)[at]
@@ -138,6 +148,11 @@ class Decoder:
     def _fits(self, tokens: int) -> None:
         if tokens > self.max_tokens:
             raise RuntimeError(f"Decoder: a row of {tokens} tokens, max_tokens is {self.max_tokens}")
+
+    def _known(self, tokens) -> None:
+        for t in tokens:
+            if not 0 <= t < self.embedding.shape[0]:
+                raise RuntimeError(f"Decoder: token {t} is outside the vocabulary of {self.embedding.shape[0]}")
 
     def _have(self, rows: Rows) -> None:
         short = int(rows.missing.item())
