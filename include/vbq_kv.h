@@ -63,7 +63,10 @@ int vbq_kv_read(const void* codes, const float* scales, int64_t pages, int32_t l
                 const int32_t* lens, const int32_t* q_start, int32_t seqs, int64_t rows, void* k_out,
                 void* v_out, int32_t dtype, void* stream);
 
-/* Workspace bytes vbq_kv_attention needs on the current device (for any batch). */
+/* What of an attention workspace has to be zero before its first use: the bytes at its beginning. */
+#define VBQ_KV_ATTENTION_ZERO_BYTES 16384
+
+/* Workspace bytes vbq_kv_attention needs on the current device (for any batch); they go by dim. */
 int vbq_kv_attention_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t dim, int32_t dtype,
                                      size_t* bytes);
 
@@ -84,8 +87,9 @@ int vbq_kv_attention_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t di
  * enter with 22 bits for fp32 and 11 (fp16) for bf16 activations.  Results are
  * deterministic.  max_new: the most new tokens any sequence has, or 0 when unknown; it
  * selects the kernel, never the result's coverage.  workspace: vbq_kv_attention_workspace_bytes() of
- * 16-byte aligned device memory, zero-filled before its first use; a call leaves what it needs to be
- * zero at zero.  Calls that may run at the same time must not share it.
+ * 16-byte aligned device memory for one value of dim, its first VBQ_KV_ATTENTION_ZERO_BYTES zeroed before
+ * its first use; a call leaves what it needs to be zero at zero.  Calls that may run at the same time must
+ * not share it.
  */
 int vbq_kv_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, float* lse,
                      int32_t dtype, int64_t rows, int32_t heads, const void* codes, const float* scales,

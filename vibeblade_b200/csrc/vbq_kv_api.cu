@@ -9,6 +9,8 @@ namespace {
 
 using vbq::api_status;
 
+static_assert(vbq::kKvHeadBytes <= VBQ_KV_ATTENTION_ZERO_BYTES, "the counters lie in what the caller zeroes");
+
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 int ok() { return api_status(VBQ_OK, nullptr); }

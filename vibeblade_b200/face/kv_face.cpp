@@ -6,9 +6,11 @@
 // vibeblade_b200/kvcache.py; each passes its arguments on by position.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <stdexcept>
@@ -105,18 +107,47 @@ int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t
 
 void* stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
-// Workspaces by (device, stream, kind, layout), zero-filled once; a call leaves zero what has to be.
-// Kept until the process ends (never destroyed: CUDA may be gone by then).
+// Workspaces by (device, stream, kind, layout, size), of which the first `zero` bytes are zeroed once; a call
+// leaves zero what has to be.  One that was handed out is never replaced or freed, because a captured graph
+// may hold its address (and never destroyed: CUDA may be gone by then).  Sizes below 1 MB, which go by a
+// call's rows, are rounded up to powers of two, so that there are few.
+//
+// A call that is captured before its stream has the workspace gets one of the graph's own: memory of the
+// graph's pool, whose zeroing is recorded and so runs at each replay.  The capture's later calls share it.
 struct Space {
   void* p;
   size_t n;
 };
-Space workspace(const at::Tensor& like, void* stream, int kind, int64_t layout, size_t need) {
-  static auto& all = *new std::map<std::tuple<int64_t, void*, int, int64_t>, at::Tensor>();
-  at::Tensor& t = all[{like.get_device(), stream, kind, layout}];
-  if (!t.defined() || (size_t)t.numel() < need)
-    t = at::zeros({(int64_t)(need < 16 ? 16 : need)}, like.options().dtype(at::kByte));
-  return {t.data_ptr(), (size_t)t.numel()};
+Space workspace(const at::Tensor& like, void* stream, int kind, int64_t layout, size_t need, size_t zero) {
+  using Key = std::tuple<int64_t, void*, int, int64_t, size_t>;
+  struct Captured {
+    unsigned long long capture;
+    at::Tensor t;
+  };
+  static auto& all = *new std::map<Key, at::Tensor>();
+  static auto& captured = *new std::map<Key, Captured>();
+  size_t size = need;
+  if (need < (1 << 20))
+    for (size = 256; size < need;) size *= 2;
+  const Key key{like.get_device(), stream, kind, layout, size};
+  const auto known = all.find(key);
+  if (known != all.end()) return {known->second.data_ptr(), size};
+  auto made = [&]() {
+    const at::Tensor t = at::empty({(int64_t)size}, like.options().dtype(at::kByte));
+    t.narrow(0, 0, (int64_t)std::min(size, zero)).zero_();
+    return t;
+  };
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &capture));
+  if (status == cudaStreamCaptureStatusNone) {
+    const at::Tensor t = made();
+    all.emplace(key, t);
+    return {t.data_ptr(), size};
+  }
+  Captured& c = captured[key];
+  if (!c.t.defined() || c.capture != capture) c = {capture, made()};
+  return {c.t.data_ptr(), size};
 }
 
 PyObject* wrap(const at::Tensor& t) { return THPVariable_Wrap(t); }
@@ -209,7 +240,7 @@ PyObject* attention(PyObject* const* a) {
   size_t need = 0;
   done(vbq_kv_attention_workspace_bytes((int32_t)heads, p.heads, p.dim, d, &need));
   void* st = stream_of(q);
-  const Space ws = workspace(q, st, 0, 0, need);
+  const Space ws = workspace(q, st, 0, p.dim, need, VBQ_KV_ATTENTION_ZERO_BYTES);  // its layout goes by dim
   done(vbq_kv_attention(q.const_data_ptr(), row_stride(q), out.data_ptr(), row_stride(out),
                         with_lse ? lse.data_ptr<float>() : nullptr, d, rows, (int32_t)heads, p.codes, p.scales, p.pages,
                         p.layers, layer, p.heads, p.page, p.dim, b.tables, b.max_pages, b.lens, b.q_start, b.seqs, scale,
@@ -234,7 +265,7 @@ Rows sequences(const char* name, const at::Tensor& refs, const at::Tensor& table
 Space pages_space(const at::Tensor& refs, void* st, int64_t pages, int32_t rows) {
   size_t need = 0;
   done(vbq_kv_pages_workspace_bytes(pages, rows, &need));
-  return workspace(refs, st, 1, pages, need);  // what stays zero is laid out by `pages`
+  return workspace(refs, st, 1, pages, need, need);  // what stays zero is laid out by `pages`
 }
 
 PyObject* reserve(PyObject* const* a) {
@@ -327,7 +358,7 @@ PyObject* logprobs(PyObject* const* a) {
   if (tok) lp = at::empty({rows}, f);
   const at::Tensor en = at::empty({rows}, f), tl = at::empty({rows, top}, f), tt = at::empty({rows, top}, f.dtype(at::kInt));
   void* st = stream_of(x);
-  const Space ws = need ? workspace(x, st, 2, 0, need) : Space{nullptr, 0};
+  const Space ws = need ? workspace(x, st, 2, 0, need, need) : Space{nullptr, 0};
   done(vbq_token_logprobs(x.const_data_ptr(), row_stride(x), d, rows, vocab, tok, top, tok ? lp.data_ptr<float>() : nullptr,
                           en.data_ptr<float>(), tl.data_ptr<float>(), tt.data_ptr<int32_t>(), ws.p, ws.n, st));
   PyObject* first = tok ? wrap(lp) : (Py_INCREF(Py_None), Py_None);

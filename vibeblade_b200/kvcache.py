@@ -16,7 +16,9 @@ are rows of ``tables`` (int32 [seqs, max_pages], page numbers, -1 for none) with
 (int32 [seqs], new ones included); ``q_start`` (int32 [seqs + 1]) says which rows of q, k and v
 are each sequence's last tokens.  ``refs`` (int32 [pages]) counts the rows that hold a page; 0
 is free.  Everything stays on the device: no call synchronises, and each may be captured in a
-CUDA graph after a first call on its stream (which makes the stream's workspace).
+CUDA graph.  Calls share workspaces by stream, which are made by the first call that needs them and
+kept; graphs captured on one stream after such a call share them too, so they are replayed one after
+the other.  A call captured before that has a workspace in its graph's own pool, cleared at each replay.
 """
 from __future__ import annotations
 
