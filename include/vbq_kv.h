@@ -66,7 +66,10 @@ int vbq_kv_read(const void* codes, const float* scales, int64_t pages, int32_t l
 /* What of an attention workspace has to be zero before its first use: the bytes at its beginning. */
 #define VBQ_KV_ATTENTION_ZERO_BYTES 16384
 
-/* Workspace bytes vbq_kv_attention needs on the current device (for any batch); they go by dim. */
+/*
+ * Workspace bytes vbq_kv_attention needs on the current device (for any batch); they go by dim.  The first
+ * VBQ_KV_ATTENTION_ZERO_BYTES are zeroed before the workspace's first use; see vbq_kv_attention.
+ */
 int vbq_kv_attention_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t dim, int32_t dtype,
                                      size_t* bytes);
 
@@ -87,9 +90,9 @@ int vbq_kv_attention_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t di
  * enter with 22 bits for fp32 and 11 (fp16) for bf16 activations.  Results are
  * deterministic.  max_new: the most new tokens any sequence has, or 0 when unknown; it
  * selects the kernel, never the result's coverage.  workspace: vbq_kv_attention_workspace_bytes() of
- * 16-byte aligned device memory for one value of dim, its first VBQ_KV_ATTENTION_ZERO_BYTES zeroed before
- * its first use; a call leaves what it needs to be zero at zero.  Calls that may run at the same time must
- * not share it.
+ * 16-byte aligned device memory, its first VBQ_KV_ATTENTION_ZERO_BYTES zeroed before its first use; a call
+ * leaves what it needs to be zero at zero, and any sizes that fit may follow one another in it.  Calls that
+ * may run at the same time must not share it.
  */
 int vbq_kv_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, float* lse,
                      int32_t dtype, int64_t rows, int32_t heads, const void* codes, const float* scales,
@@ -98,7 +101,13 @@ int vbq_kv_attention(const void* q, int64_t q_stride, void* out, int64_t out_str
                      const int32_t* q_start, int32_t seqs, float scale, int32_t window, int32_t max_new,
                      void* workspace, size_t workspace_bytes, void* stream);
 
-/* Workspace bytes the page moves below need for a pool of `pages` pages and `rows` sequences. */
+/*
+ * Workspace bytes the page moves below need for a pool of `pages` pages and `rows` sequences (of
+ * vbq_kv_fork the larger of rows and new_rows).  The workspace is 16-byte aligned device memory, zero-filled
+ * before its first use and again before it serves a pool of another number of pages (what a fork needs to
+ * be zero lies by `pages`); every call leaves that at zero.  Calls that may run at the same time must not
+ * share it.
+ */
 int vbq_kv_pages_workspace_bytes(int64_t pages, int32_t rows, size_t* bytes);
 
 /*
@@ -138,7 +147,11 @@ int vbq_kv_compact(void* codes, float* scales, int64_t pages, int64_t page_bytes
                    int32_t rows, int32_t max_pages, int32_t* refs_out, int32_t* tables_out, int32_t* live,
                    void* workspace, size_t workspace_bytes, void* stream);
 
-/* Workspace bytes vbq_token_logprobs needs for these sizes on the current device. */
+/*
+ * Workspace bytes vbq_token_logprobs needs for these sizes on the current device.  The workspace is 16-byte
+ * aligned device memory, zero-filled before its first use; any sizes that fit may follow one another in it.
+ * Calls that may run at the same time must not share it.
+ */
 int vbq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top, size_t* bytes);
 
 /*
@@ -151,7 +164,7 @@ int vbq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top,
  * one pass over the logits, sums in fp32.  -inf logits have probability 0; a row of nothing
  * but -inf has logprob and top_logprob -inf and entropy 0; a row with NaN or +inf has NaN
  * logprob and entropy.  tokens may be NULL (then logprob is not written), entropy may be
- * NULL.  workspace as for vbq_kv_attention.
+ * NULL.
  */
 int vbq_token_logprobs(const void* logits, int64_t stride, int32_t dtype, int64_t rows, int64_t vocab,
                        const int32_t* tokens, int32_t top, float* logprob, float* entropy,
