@@ -12,7 +12,7 @@
  *     scales  fp32 [pages][layers][2][kv_heads]
  * A stored value is scale * code.  `page` tokens (16, 32, 64 or 128) of one head share a
  * scale; dim is 64, 128 or 256.  A page is one contiguous run over every layer, so moving a
- * page is one copy.  Codes must be 16-byte aligned, scales 4-byte aligned.
+ * page is one copy.  Codes must be 16-byte aligned, scales and every int32 and fp32 array 4-byte aligned.
  *
  * A batch of sequences is described by three device arrays:
  *     tables  int32 [seqs][max_pages]  the page of each run of `page` tokens (-1: none)

@@ -13,6 +13,10 @@ static_assert(vbq::kKvHeadBytes <= VBQ_KV_ATTENTION_ZERO_BYTES, "the counters li
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// int32 and fp32 arrays; those that may be NULL are aligned then
+template <typename... P> bool words(const P*... p) { return (aligned(p, 4) && ...); }
+int bad_words(const char* who) { return api_status(VBQ_ERR_ALIGN, "%s: the int32 and fp32 arrays must be 4-byte aligned", who); }
+
 int ok() { return api_status(VBQ_OK, nullptr); }
 int launched(const char* who, cudaError_t e) {
   return e == cudaSuccess ? ok() : api_status(VBQ_ERR_CUDA, "%s launch: %s", who, cudaGetErrorString(e));
@@ -193,6 +197,7 @@ int vbq_kv_reserve(const int32_t* refs, const int32_t* tables, const int32_t* le
   if (int rc = pool_sizes(who, pages, page, rows, max_pages)) return rc;
   if (!refs || !refs_out || !missing || (rows > 0 && (!tables || !lens || !new_tokens || !tables_out || !lens_out)))
     return api_status(VBQ_ERR_NULL, "%s: NULL pointer", who);
+  if (!words(refs, tables, lens, new_tokens, refs_out, tables_out, lens_out, missing)) return bad_words(who);
   if (int rc = workspace_ok(who, workspace, workspace_bytes, vbq::kv_pages_workspace(pages, rows))) return rc;
   return launched(who, vbq::launch_kv_reserve(refs, tables, lens, new_tokens, pages, page, rows, max_pages, refs_out,
                                               tables_out, lens_out, missing, workspace,
@@ -213,6 +218,7 @@ int vbq_kv_fork(void* codes, float* scales, int64_t pages, int64_t page_bytes, i
     return api_status(VBQ_ERR_NULL, "%s: NULL pointer", who);
   if ((new_rows > 0 && rows > 0) && (tables_out == tables || lens_out == lens))
     return api_status(VBQ_ERR_SHAPE, "%s: tables_out and lens_out must not be tables and lens", who);
+  if (!words(refs, tables, lens, parents, refs_out, tables_out, lens_out, missing)) return bad_words(who);
   const int32_t most = rows > new_rows ? rows : new_rows;
   if (int rc = workspace_ok(who, workspace, workspace_bytes, vbq::kv_pages_workspace(pages, most))) return rc;
   const vbq::KvPool pool{static_cast<uint8_t*>(codes), scales, pages, page_bytes, page_scales, page};
@@ -230,6 +236,7 @@ int vbq_kv_compact(void* codes, float* scales, int64_t pages, int64_t page_bytes
   if (int rc = pool_data(who, codes, scales, page_bytes, page_scales)) return rc;
   if (!refs || !refs_out || !live || (rows > 0 && (!tables || !lens || !tables_out)))
     return api_status(VBQ_ERR_NULL, "%s: NULL pointer", who);
+  if (!words(refs, tables, lens, refs_out, tables_out, live)) return bad_words(who);
   if (int rc = workspace_ok(who, workspace, workspace_bytes, vbq::kv_pages_workspace(pages, rows))) return rc;
   const vbq::KvPool pool{static_cast<uint8_t*>(codes), scales, pages, page_bytes, page_scales, page};
   return launched(who, vbq::launch_kv_compact(pool, refs, tables, lens, rows, max_pages, refs_out, tables_out, live,
@@ -265,6 +272,7 @@ int vbq_token_logprobs(const void* logits, int64_t stride, int32_t dtype, int64_
     return api_status(VBQ_ERR_NULL, "%s: NULL pointer", who);
   if (!aligned(logits, dtype == VBQ_DTYPE_F32 ? 4 : 2))
     return api_status(VBQ_ERR_ALIGN, "%s: logits must be element-aligned", who);
+  if (!words(tokens, logprob, entropy, top_logprob, top_token)) return bad_words(who);
   if (int rc = workspace_ok(who, workspace, workspace_bytes, vbq::logprobs_workspace(rows, vocab, top))) return rc;
   return launched(who, vbq::launch_logprobs(logits, stride, dtype == VBQ_DTYPE_BF16, rows, vocab, tokens, top, logprob,
                                             entropy, top_logprob, top_token, workspace,
