@@ -32,3 +32,13 @@ def test_asynchronous_copies_are_ordered_for_the_compiler(name):
     compiler may move reads of the copied bytes above the wait."""
     loose = [s for s in statements((CSRC / name).read_text()) if "cp.async" in s and '"memory"' not in s]
     assert not loose, loose
+
+
+@pytest.mark.parametrize("name", FILES)
+def test_waits_are_bounded_in_time(name):
+    """A loop over mbarrier tries looks at the clock (how long a try is suspended is the hardware's choice,
+    so a number of tries bounds nothing), or at a flag that one which does raises."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+    loops = [text[m.start():m.start() + 200] for m in re.finditer(r"while \(!mbar_try_wait\w*\(", text)]
+    timed = [t for t in loops if "clock" in t]
+    assert all(t in timed or (timed and "abort_flag" in t) for t in loops), loops

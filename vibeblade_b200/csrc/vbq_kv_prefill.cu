@@ -36,9 +36,10 @@
 // against 2.01; scores in two products of 64 tokens, the first early, 2.15 (an MMA of 64 columns
 // takes as long as one of 128); a quarter of the exponentials as polynomials, 2.29.
 //
-// Every mbarrier wait is bounded; one that gives up raises the device status word and an
-// abort flag at which every later wait returns at once and no MMA is issued, so the roles run
-// out of their (finite) schedules and tensor memory is freed.
+// Every mbarrier wait is bounded in time: the schedule's warp waits for each piece's end by the clock, and
+// where it gives up raises the device status word and an abort flag at which every wait returns at once
+// and no MMA is issued, so the roles run out of their (finite) schedules, what was issued is waited for,
+// and tensor memory is freed.
 #include <cmath>
 
 #include "vbq_internal.h"
@@ -63,6 +64,7 @@ struct PBars {
   uint64_t scale_full[kScaleRing], scale_empty[kScaleRing];
   uint64_t seg_full[2], seg_empty[2];
   uint64_t part_a, part_b;
+  uint64_t drain;  // after an abort: what was issued has ended
   int64_t runs[16];  // of each warp's sequences
   int longest[16];
   uint32_t tmem;
@@ -331,8 +333,9 @@ struct PWalk {
   int whole_upto;
 };
 
-// Tries of a wait before it gives up: each is at least some tens of cycles, so most of a second.
-constexpr int kTries = 1 << 25;
+// SM clock cycles after which the watch gives up, 1.5 s at 1.965 GHz (of the clock's low word, which comes
+// round every 2^32 and is looked at far more often), for every 2^14 runs a CTA's pieces may have.
+constexpr uint32_t kWatchCycles = 3000000000u;
 
 template <int D> constexpr int p_part_floats() { return kTileRows * (D + 2); }  // O [D / 4][256][4], m, l
 
@@ -372,6 +375,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
     }
     mbar_init(smem_u32(&bars.part_a), 8);
     mbar_init(smem_u32(&bars.part_b), 1);
+    mbar_init(smem_u32(&bars.drain), 1);
     bars.abort = 0;
     mbar_fence_init();
   }
@@ -406,16 +410,14 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
   p_fence_after();
   const uint32_t tmem = __shfl_sync(kFull, bars.tmem, 0);
   volatile int* abort_flag = &bars.abort;
-  // After a wait gives up every later one returns at once.
+  // A wait ends with the abort flag too, which the schedule's warp raises: whatever stalls, a piece does not
+  // end, and that warp waits for each piece's end by the clock.  (These waits are many and their code is
+  // short for the instruction cache: with a clock in each, short prompts took 122 us instead of 111.)
   auto wait = [&](uint64_t& bar, uint32_t parity) {
     const uint32_t addr = smem_u32(&bar);
-    int n = 0;
 #pragma unroll 1
-    while (!mbar_try_wait(addr, parity) && !*abort_flag)
-      if (++n == kTries) {
-        *abort_flag = 1;
-        g_kv_prefill_status = kStatusTimeout;
-      }
+    while (!mbar_try_wait(addr, parity) && !*abort_flag) {
+    }
   };
   // the next piece, for a role that has done k pieces; false when there is none
   auto piece = [&](uint32_t k) {
@@ -862,13 +864,19 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
         }
         piece_done(k);
       }
-      // the last commits of the K and V stages have arrived before the CTA may leave
-      if (count > 0 && !aborted()) {
+      // What was issued has ended, and its commits have arrived, before tensor memory is freed and the CTA
+      // leaves: after an abort through a commit of its own.  Nobody watches any more: these go by the clock.
+      bool ended = true;
+      if (aborted()) {
+        p_commit(lead, smem_u32(&bars.drain));
+        ended = mbar_wait_bounded(smem_u32(&bars.drain), 0, kWaitBudgetCycles);
+      } else if (count > 0) {
         for (uint32_t k = count > 2 ? count - 2 : 0; k < count; ++k) {
-          wait(bars.k_empty[k & 1], (k >> 1) & 1);
-          wait(bars.v_empty[k & 1], (k >> 1) & 1);
+          ended = mbar_wait_bounded(smem_u32(&bars.k_empty[k & 1]), (k >> 1) & 1, kWaitBudgetCycles) && ended;
+          ended = mbar_wait_bounded(smem_u32(&bars.v_empty[k & 1]), (k >> 1) & 1, kWaitBudgetCycles) && ended;
         }
       }
+      if (!ended) g_kv_prefill_status = kStatusTimeout;
     } else if (warp == 14) {
       // ------------------------------ scales ------------------------------
       uint32_t count = 0;
@@ -913,9 +921,23 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
       int longest = 0;
       for (int i = 0; i < kPThreads / 32; ++i) total += bars.runs[i], longest = max(longest, bars.longest[i]);
       w.init(b, a, c.heads, lane, runs, total, longest);
+      // waits for a piece's end; false, and the whole CTA is given up, where that does not come
+      auto watch = [&](uint64_t& bar, uint32_t parity) {
+        const uint32_t addr = smem_u32(&bar);
+        int64_t times = 1 + (w.per >> 14);
+        uint32_t since = clock();
+#pragma unroll 1
+        while (!mbar_try_wait(addr, parity) && !*abort_flag) {
+          if ((uint32_t)clock() - since <= kWatchCycles) continue;
+          since = clock();
+          if (--times > 0) continue;
+          *abort_flag = 1;
+          g_kv_prefill_status = kStatusTimeout;
+        }
+        return !__any_sync(kFull, *abort_flag);
+      };
       uint32_t k = 0;
-      for (; w.more() && !*abort_flag; w.next(b, a, c.heads, runs), ++k) {
-        wait(bars.seg_empty[k & 1], ((k >> 1) & 1) ^ 1);
+      for (; w.more() && watch(bars.seg_empty[k & 1], ((k >> 1) & 1) ^ 1); w.next(b, a, c.heads, runs), ++k) {
         if (lane == 0) {
           PSeg g;
           g.s = w.s, g.head = w.head, g.tile = w.tile, g.c0 = w.c0, g.c1 = w.c1, g.first = w.run.first;
@@ -928,11 +950,12 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
         }
         __syncwarp();
       }
-      wait(bars.seg_empty[k & 1], ((k >> 1) & 1) ^ 1);
+      watch(bars.seg_empty[k & 1], ((k >> 1) & 1) ^ 1);
       if (lane == 0) {
         segs[k & 1].stop = 1;
         mbar_arrive(smem_u32(&bars.seg_full[k & 1]));
       }
+      if (k > 0) watch(bars.seg_empty[(k - 1) & 1], ((k - 1) >> 1) & 1);  // the last piece's
     }
   }
   p_fence_before();
