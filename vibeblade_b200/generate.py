@@ -9,7 +9,8 @@ and fp32 keys and values on the host):
     lm_head -> token_logprobs      log probabilities and the likeliest tokens
     kv_fork                        rows regrouped by the beams that live on
 
-Rows are sequences; every tensor of the loop stays on the device and no step waits for it.
+Rows are sequences; every tensor of the loop stays on the device and no step waits for it (score and
+beam_search wait once, for the count of missing pages).
 
     dec = Decoder(layers, embedding, final_norm, (lm_head, type, vocab), pages=512)
     logprobs = dec.score([prompt_a, prompt_b])
@@ -65,6 +66,11 @@ class Decoder:
         z = lambda *s: torch.zeros(s, dtype=torch.int32, device=self.dev)  # noqa: E731
         return Rows(z(self.codes.shape[0]), z(n, self.max_pages) - 1, z(n), z(1))
 
+    def _sent(self, values: list[int], dtype: torch.dtype = torch.int32) -> torch.Tensor:
+        """A host list on the device, without waiting for it (a copy from pageable memory waits)."""
+        t = torch.tensor(values, dtype=dtype)
+        return t.pin_memory().to(self.dev, non_blocking=True) if self.dev.type == "cuda" else t
+
     def _rope(self, x: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
         """Rotate the halves of each head (vibeblade/transformer.py:73-99); at [T]: positions."""
         dim = self.cfg.head_dim
@@ -77,7 +83,7 @@ class Decoder:
         """Append ``new[r]`` tokens to each row (``tokens`` [sum(new)], row after row) and run the
         blocks on them.  Returns the rows and the last block's output [sum(new), hidden].  Tokens past
         a row's pages count in ``missing`` and are not stored."""
-        n = torch.tensor(new, dtype=torch.int32, device=self.dev)
+        n = self._sent(new)
         q_start = torch.zeros(len(new) + 1, dtype=torch.int32, device=self.dev)
         torch.cumsum(n, 0, out=q_start[1:])
         refs, tables, lens, missing = kv_reserve(rows.refs, rows.tables, rows.lens, n, self.page)
@@ -109,11 +115,11 @@ class Decoder:
         self._known(t for p in prompts for t in p)
         if sum(new) == 0:
             return [torch.empty(0, device=self.dev) for _ in prompts]
-        tokens = torch.tensor([t for p in prompts for t in p], device=self.dev)
+        tokens = self._sent([t for p in prompts for t in p], torch.long)
         rows, x = self.forward(self.rows(len(prompts)), tokens, new)
         self._have(rows)
         # row i predicts token i + 1; a prompt's last row has no token to score
-        nxt = torch.tensor([t for p in prompts for t in (*p[1:], -1)], dtype=torch.int32, device=self.dev)
+        nxt = self._sent([t for p in prompts for t in (*p[1:], -1)])
         logprob = token_logprobs(self.logits(x), nxt)[0]
         return [lp[:-1] for lp in torch.split(logprob, new)]
 
@@ -127,7 +133,7 @@ class Decoder:
             raise RuntimeError("Decoder: the prompt is empty")
         self._known(prompt)
         self._fits(len(prompt) + max(steps - 1, 0))  # the last tokens are not run
-        rows, x = self.forward(self.rows(1), torch.tensor(prompt, device=dev), [len(prompt)])
+        rows, x = self.forward(self.rows(1), self._sent(prompt, torch.long), [len(prompt)])
         logits = self.logits(x[-1:])
         total = torch.zeros(1, device=dev)
         out = torch.empty((1, 0), dtype=torch.int32, device=dev)
