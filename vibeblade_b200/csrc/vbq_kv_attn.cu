@@ -104,7 +104,7 @@ template <int D, int NT> struct Part {  // one CTA's part of a group, in the wor
 constexpr int kDigits = 3;
 // Resident CTAs the registers are held to.  Three of dim 128 (166 registers) beat four (128): 142 us
 // against 156 over 762 MB.
-template <int D, int NT> constexpr int resident_of() { return D == 256 || NT > 1 && D == 128 ? 2 : NT > 1 || D == 128 ? 3 : 4; }
+template <int D, int NT> constexpr int resident_of() { return D == 256 || NT > 1 && D == 128 ? 2 : NT > 1 || D == 128 ? 3 : kKvMaxResident; }
 
 // Shared memory of a CTA: each warp's ring of blocks (16 tokens of K and V and the two scales),
 // then the query digits and the warps' maxima and sums.  What the ring is for is loads in flight,

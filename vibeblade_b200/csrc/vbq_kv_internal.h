@@ -41,8 +41,9 @@ struct KvAttention {
   // a launch takes the sequences whose rows (new tokens times group) are in (rows_above, rows_upto]
   int64_t rows_above, rows_upto;
 };
-constexpr int kKvCounterBytes = 4 * 16 * 148;  // the attention workspace's zeroed head
 constexpr int kKvMaxSms = 148;
+constexpr int kKvMaxResident = 4;  // CTAs an SM of the kernel for few rows
+constexpr int kKvCounterBytes = 4 * kKvMaxResident * kKvMaxSms;  // the attention workspace's zeroed head
 constexpr int kKvHeadBytes = kKvCounterBytes + 4 * kKvMaxSms;  // with the tile kernel's counters
 size_t kv_attn_tile_parts(int dim);  // where in the workspace the tile kernel's parts begin
 // Split over the cache's tokens (vbq_kv_attn.cu): any type, any number of new tokens.
