@@ -40,8 +40,10 @@ def _weights_u8(w: torch.Tensor) -> torch.Tensor:
 
 
 # Zero-filled split-K scratch per (device, stream).  Calls on one stream run in order,
-# and every call leaves the buffer zero-filled again, so one buffer per stream is safe.
+# and every call leaves the buffer zero-filled again, so one buffer per stream is safe.  A
+# buffer that a larger one takes the place of is kept: a captured graph may hold its address.
 _SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+_SCRATCH_BEFORE: list[torch.Tensor] = []
 
 
 _CUDA_AVAILABLE: list[bool] = []
@@ -80,6 +82,9 @@ def _stream_scratch(device: torch.device, stream: int, nbytes: int) -> torch.Ten
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
     buf = _SCRATCH.get(key)
     if buf is None or buf.numel() < nbytes:
+        if buf is not None:
+            _SCRATCH_BEFORE.append(buf)
+            nbytes = max(nbytes, 2 * buf.numel())  # so that few are kept
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _SCRATCH[key] = buf
     return buf
