@@ -369,8 +369,8 @@ logprobs_kernel(const void* __restrict__ logits, int64_t stride, int64_t vocab, 
   // is masked come here, so the slice is summed once more, element by element.
   if (fabsf(s.r) >= kFar && fabsf(s.r) < INFINITY) {
     Sums t{s.r, 0.0f, 0.0f};
-    for (int e = x_row.e0 + tid; e < x_row.e1; e += kThreads) {
-      const float d = x_row.one(e) - s.r;
+    for (int64_t i = (int64_t)x_row.e0 + tid; i < x_row.e1; i += kThreads) {
+      const float d = x_row.one((int)i) - s.r;
       const float y = ex2(d * kLog2e);  // 0 for -inf, NaN for NaN
       t.z += y;
       if (y > 0.0f) t.b = fmaf(d, y, t.b);
