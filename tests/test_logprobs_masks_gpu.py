@@ -68,3 +68,48 @@ def test_logits_at_both_ends_of_fp32(cuda, rows):
     near(en, np.full(rows, math.log(2)))
     near(tl, np.full((rows, 2), -math.log(2)))
     assert ti[0].tolist() == [17, 4100]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows", [2, 600])
+@pytest.mark.parametrize("off", [0, 3])
+def test_lists_that_overflow(cuda, dtype, rows, off):
+    """More elements reach the list's bound than it holds: large logits crowded into the vectors of a few
+    threads, in falling and in rising order, beside ties, and ties at the row's end."""
+    V = 40003
+    r = np.random.default_rng(rows + off)
+    big = torch.from_numpy(r.normal(0, 1, (rows, V + 8)).astype(np.float32)).to(dtype).to(cuda)
+    x = big[:, off:off + V]
+    at = torch.arange(V, device=cuda) + off
+    per = 512 if rows > 512 else 256
+    lanes = (at // (8 if dtype == torch.bfloat16 else 4)) % per < 6  # of six threads, or about
+    n = int(lanes.sum())
+    steps = torch.arange(n, device=cuda, dtype=torch.float32)
+    for edit in range(5):
+        y = x.clone()
+        if edit == 0:
+            y[:, lanes] = (100 + steps / 16).to(dtype)
+        elif edit == 1:
+            y[:, lanes] = (100 - steps / 16).to(dtype)
+        elif edit == 2:
+            y[:, lanes] = (100 + (steps * 7919 % 97)).to(dtype)
+        elif edit == 3:
+            y[:] = -math.inf
+            y[:, -40:] = 1.0
+            y[:, 100] = 2.0
+        else:
+            y[:] = -math.inf
+            y[:, 7] = 3.0
+            y[:, -5:] = torch.tensor([1.0, 2.0, 1.0, 2.0, 1.0], device=cuda).to(dtype)
+            y[:, 9000] = math.nan
+        if edit == 4:  # a NaN spoils the sums, not the list
+            ti = vb.token_logprobs(y, None, 9)[3]
+            want = [7, V - 4, V - 2, V - 5, V - 3, V - 1, 0, 1, 2]
+            assert (ti.cpu() == torch.tensor(want, dtype=torch.int32)).all()
+            continue
+        for top in (1, 20, 32):
+            got = vb.token_logprobs(y, None, top)
+            _, en, tl, ti = plain(y[:2].double().cpu().numpy(), None, top)
+            assert np.array_equal(got[3][:2].cpu().numpy(), ti)
+            near(got[2][:2], tl)
+            near(got[1][:2], en)

@@ -10,8 +10,9 @@
 // few largest) is at most the top-th largest logit.  Only lanes whose maximum reaches that bound
 // can hold one of the top (not many more than `top`), and only their elements are read again, by
 // the whole warp, 32 vectors at a time; the elements that reach the bound are collected in shared
-// memory and ranked by counting (value, then lower token).  Rows with more such elements than fit
-// (a great many equal logits) take a plain insertion scan.
+// memory and ranked by counting (value, then lower token).  Where more of them reach it than fit (a mask
+// that leaves fewer tokens than are listed: the bound is then the mask's value) the row is read twice
+// more: for what lies above the bound, and up to the first of its equals that are wanted.
 //
 // Few long rows are split over CTAs; the last to arrive joins the slices' sums in slice order
 // and ranks their top lists the same way.
@@ -163,6 +164,84 @@ __device__ __forceinline__ void insert(float x, int i, bool want, int top, int l
   }
 }
 
+// The list of a slice of which more elements reach the bound than the shared list holds: those above it,
+// by rank, then its equals, lowest first.  Too many above it (large logits crowded into few lanes): the
+// top-th of as many as fit is a bound too, and a higher one; after kRaises such passes one warp inserts
+// the elements one by one.
+constexpr int kRaises = 8;
+template <bool BF16, int kThreads>
+__device__ __forceinline__ void crowded(Shared<kThreads>& sh, const Row<BF16> row, float bound, int top) {
+  constexpr int kN = Row<BF16>::kN, kWarps = kThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto above = [&](float x, int e) {
+    if (x > bound) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCap) sh.cv[at] = x, sh.ci[at] = e;
+    }
+  };
+  int n;
+  for (int raise = 0;; ++raise) {
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    for (int a = row.a0 + tid; a < row.a1; a += kThreads) {
+      float x[kN];
+      row.unpack(row.vec(a), x);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) above(x[j], a * kN - row.lead + j);
+    }
+    if (tid < 2 * kN && row.loose(tid) >= 0) above(row.one(row.loose(tid)), row.loose(tid));
+    __syncthreads();
+    n = sh.count;
+    if (n <= kCap || raise == kRaises) break;
+    for (int a = tid; a < kCap; a += kThreads) {
+      int r = 0;
+      for (int c = 0; c < kCap; ++c) r += better(sh.cv[c], sh.ci[c], sh.cv[a], sh.ci[a]);
+      if (r == top - 1) sh.bound_f = sh.cv[a];
+    }
+    __syncthreads();
+    bound = sh.bound_f;
+  }
+  if (n > kCap) {
+    if (warp == 0) {
+      float lv = -INFINITY;
+      int li = INT_MAX;
+      for (int64_t a = row.e0; a < row.e1; a += 32) {
+        const bool in = a + lane < row.e1;
+        insert(in ? row.one((int)a + lane) : 0.0f, (int)a + lane, in, top, lane, lv, li);
+      }
+      if (lane < top) sh.tv[lane] = lv, sh.ti[lane] = li;
+    }
+    return;
+  }
+  rank_candidates(sh, n, top);
+  // kEach elements a thread, in order
+  constexpr int kEach = 8;
+  int* counts = reinterpret_cast<int*>(sh.tops);
+  for (int64_t e0 = row.e0; e0 < row.e1 && n < top; e0 += kThreads * kEach) {
+    const int64_t e = e0 + tid * kEach;
+    unsigned equal = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (e + j < row.e1 && row.one((int)(e + j)) == bound) equal |= 1u << j;
+    const int upto = kv::warp_scan(__popc(equal), lane);
+    if (lane == 31) counts[warp] = upto;
+    __syncthreads();
+    int r = n + upto - __popc(equal), all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) r += counts[w];
+      all += counts[w];
+    }
+    for (; equal && r < top; ++r, equal &= equal - 1) {
+      const int i = (int)e + __ffs(equal) - 1;
+      sh.tv[r] = row.one(i), sh.ti[r] = i;
+    }
+    n += all;
+    __syncthreads();
+  }
+}
+
 // Writes a row's results from its sums (in sh.part[0]) and its top list.
 template <int kThreads>
 __device__ __forceinline__ void finish(Shared<kThreads>& sh, const Sums& s, float x_token, bool has_token, bool counted, int64_t row,
@@ -309,7 +388,9 @@ logprobs_kernel(const void* __restrict__ logits, int64_t stride, int64_t vocab, 
     __syncthreads();
     const float bound = sh.bound_f;
     unsigned flagged = __ballot_sync(kFull, mx >= bound);
+    volatile int* found = &sh.count;
     auto candidate = [&](float x, int e) {
+      if (*found > kCap) return;
       const int at = atomicAdd(&sh.count, 1);
       if (at < kCap) sh.cv[at] = x, sh.ci[at] = e;
     };
@@ -332,7 +413,7 @@ logprobs_kernel(const void* __restrict__ logits, int64_t stride, int64_t vocab, 
           if (x[j] >= bound) candidate(x[j], a * kN - x_row.lead + j);
       }
     }
-    while (flagged) {
+    while (flagged && *found <= kCap) {
       const int l = __ffs(flagged) - 1;
       flagged &= flagged - 1;
       for (int a = few ? x_row.a1 : x_row.a0 + (warp * 32 + l) + lane * kThreads; a < x_row.a1; a += 32 * kThreads) {
@@ -348,17 +429,8 @@ logprobs_kernel(const void* __restrict__ logits, int64_t stride, int64_t vocab, 
       }
     }
     __syncthreads();
-    if (sh.count <= kCap) {
-      rank_candidates(sh, sh.count, top);
-    } else if (warp == 0) {
-      float lv = -INFINITY;
-      int li = INT_MAX;
-      for (int a = x_row.e0; a < x_row.e1; a += 32) {
-        const bool in = a + lane < x_row.e1;
-        insert(in ? x_row.one(a + lane) : 0.0f, a + lane, in, top, lane, lv, li);
-      }
-      if (lane < top) sh.tv[lane] = lv, sh.ti[lane] = li;
-    }
+    if (sh.count <= kCap) rank_candidates(sh, sh.count, top);
+    else crowded<BF16, kThreads>(sh, x_row, bound, top);
     __syncthreads();
   }
   s = sh.part[0];
