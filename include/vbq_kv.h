@@ -10,8 +10,8 @@
  * The cache is two caller-owned device buffers:
  *     codes   int8 [pages][layers][2][kv_heads][page][dim]     (2: keys, then values)
  *     scales  fp32 [pages][layers][2][kv_heads]
- * A stored value is scale * code.  `page` tokens (16, 32, 64 or 128) of one head share a
- * scale; dim is 64, 128 or 256.  A page is one contiguous run over every layer, so moving a
+ * A stored value is scale * code, scales finite and not negative.  `page` tokens (16, 32, 64 or 128)
+ * of one head share a scale; dim is 64, 128 or 256.  A page is one contiguous run over every layer, so moving a
  * page is one copy.  Codes must be 16-byte aligned, scales and every int32 and fp32 array 4-byte aligned.
  *
  * A batch of sequences is described by three device arrays:
@@ -46,8 +46,8 @@ extern "C" {
  *     old codes become rint(code * (s0 / s1)) when s1 > s0
  *     new codes are rint(x / s1) clamped to +-127
  * in fp32 with one rounding an operation, ties to even.  Infinities take the code +-127, NaN
- * takes 0, and neither enters the scale.  The pages must be in the tables already
- * (vbq_kv_reserve); repeating a call leaves the cache as it is.
+ * takes 0, and neither enters the scale; where s1 is 0 every new code is.  The pages must be in the
+ * tables already (vbq_kv_reserve); repeating a call leaves the cache as it is.
  */
 int vbq_kv_append(const void* k, int64_t k_stride, const void* v, int64_t v_stride, int32_t dtype,
                   int64_t rows, void* codes, float* scales, int64_t pages, int32_t layers, int32_t layer,

@@ -10,7 +10,7 @@
 //
 // Bytes bound the long appends: the rows are read once and held on chip between the look for the
 // largest value and the rounding.  Measured (device time, append and read back): 6 sequences of up
-// to 5001 new tokens, 8 heads of 128, bf16, 150 MB: 38 us, 3.9 TB/s (append 23, read 15), 70 % of
+// to 5001 new tokens, 8 heads of 128, bf16, 150 MB: 39 us, 3.9 TB/s (append 22.5, read 16.5), 70 % of
 // its issue slots taken; 64 sequences of one token, fp32: 9 us, which is latency.
 #include "vbq_internal.h"
 #include "vbq_kv.cuh"

@@ -29,12 +29,15 @@
 // workspace and the last to arrive adds them up in range order, so the result does not depend
 // on timing.
 //
-// Measured (device time of a launch): 64 sequences of up to 5003 tokens, 32 query heads over 8
-// of 128, bf16, 371 MB of codes: 80 us, 4.6 TB/s.  4 of up to 131072, 64 over 8 heads, fp32, 762
-// MB: 142 us, 5.4 TB/s; its copies alone, without the arithmetic, take 136 us.  One sequence of
-// 333 tokens: 9 us.  What the shorter ones lack is the way to the first block (plan, page
-// number, block: 4 to 8 us), the joining of parts (3 to 5 us), and CTAs of one SM that end up to
-// a fifth apart; half of the issue slots are taken.
+// Measured (device time of a launch among others): 64 sequences of up to 5003 tokens, 32 query heads
+// over 8 of 128, bf16, 371 MB of codes: 87 us at 1807 MHz, where the power limit holds the SMs in a long
+// row of calls, 80 at 1965; 4.3 and 4.6 TB/s.  4 of up to 131072, 64 over 8 heads, fp32, 762 MB: 173 us
+// at 1635 MHz, 143 at 1965; 4.4 and 5.3 TB/s; at 1965 its copies alone, without the arithmetic, take
+// 136.  One sequence of 333 tokens: 9.4 us.  What the shorter ones lack is the way to the first block
+// (plan, page number, block: 4 to 8 us), the joining of parts (3 to 5 us), and CTAs of one SM that end up
+// to a fifth apart; half of the issue slots are taken.  fp32 prompts and those with heads of 256 are this
+// kernel's too, in tiles of 16 and 8 rows that each read and turn the codes again: four prompts of 1023
+// tokens and less, 73 GFLOP, 785 us in fp32, 746 with heads of 256 in bf16.
 #include <cmath>
 
 #include "vbq_internal.h"
@@ -677,7 +680,7 @@ size_t kv_attn_workspace(int dim) {
 // of 128: 36 rows 76 us here and 95 there, 68 rows 117 and 91, 132 rows 196 and 91; 4 heads of 64 in a
 // window of 2050: 119 rows 35 and 36, 231 rows 53 and 43; 8 of 38000, one head of 64: 119 rows 48 and
 // 68, 231 rows 76 and 69; 16 of 7001, 4 heads of 64 in a window of 2050, 161 rows 42 and 53.  With few rows in all the tiles do not fill the GPU: one sequence of 3000
-// tokens, 8 heads of 128: 132 rows 30 us here and 35 there.
+// tokens, 8 heads of 128: 132 rows 30 us here and 35 there.  (All at 1965 MHz.)
 static int64_t tile_rows_from(int dim, int64_t rows) { return dim == 64 ? 192 : rows <= 2048 ? 144 : 64; }
 
 cudaError_t launch_kv_attn(const KvAttention& a0, const KvCache& c, const KvBatch& b, bool bf16, int max_new,

@@ -25,9 +25,10 @@
 // two into fp16's range, which keeps all of bf16's digits down to 2^-29 of its largest value (and
 // more coarsely 2^-39); weights are rounded to fp16's 11 bits, where the output keeps 8.
 //
-// Measured (device time of a launch, 8 heads of 128): the last 2048 of 32768 tokens of 64
-// query heads, 2.13 TFLOP: 2.03 ms, 1.05 PFLOP/s; four prompts of 1023 tokens and less, 32 query
-// heads, 73 GFLOP: 109 us, 0.67 PFLOP/s.  A run of 128 tokens takes some 4200 cycles where its MMAs
+// Measured (device time of a launch among others, 8 heads of 128): the last 2048 of 32768 tokens of 64
+// query heads, 2.13 TFLOP: 2.38 ms at 1627 MHz, where the power limit holds the SMs in a row of calls,
+// 0.90 PFLOP/s; a call by itself 2.07 ms, 1.03; four prompts of 1023 tokens and less, 32 query heads, 73
+// GFLOP: 112 us at 1965 MHz, 0.65 PFLOP/s.  A run of 128 tokens takes some 4200 cycles where its MMAs
 // need 2120 and the exponentials 2048 of the MUFU: a half's softmax is a chain of 3000 (load of S 300,
 // largest 300, 64 exponentials 900, P out 250, 64 more 900, P out), after which its second product
 // and next scores take 1050, and the halves hide only part of each other.  A tile costs 10000 to

@@ -17,10 +17,12 @@
 // Few long rows are split over CTAs; the last to arrive joins the slices' sums in slice order
 // and ranks their top lists the same way.
 //
-// Measured (device time): 2047 rows of 128256 bf16 logits, top 20, 525 MB: 114 us, 4.6 TB/s (of its
-// issue slots 71 % are taken, of the MUFU's 60 %; the rest is each row's list, under which the other
-// CTAs of the SM load); 8 rows of fp32, top 5: 11 us, which is latency: the
-// pass, the list's second reads, the join.
+// Measured (device time of a call among others): 2047 rows of 128256 bf16 logits, top 20, 525 MB: 132 us
+// at 1747 MHz, where the power limit holds the SMs in a row of calls, 4.0 TB/s; 117 at 1965 (of its issue
+// slots 69 % are taken, of the MUFU's 58 %; the rest is each row's list, under which the other CTAs of the
+// SM load).  1023 rows of fp32, as many bytes: 122 us at 1852 MHz.  600 rows of bf16, 154 MB: 47 us; 83
+// where a mask leaves three tokens a row.  8 rows of fp32, top 5: 11 us, which is latency: the pass, the
+// list's second reads, the join.
 #include <climits>
 #include <cmath>
 
@@ -563,8 +565,8 @@ cudaError_t launch_logprobs(const void* logits, int64_t stride, bool bf16, int64
   const int64_t per = ((vocab + splits - 1) / splits + 7) / 8 * 8;
   int* counters = static_cast<int*>(workspace);
   float* slices = reinterpret_cast<float*>(counters + lp::kMaxSplitRows);
-  // rows that fill the GPU by themselves: 512 threads a row (2047 rows of 128256: 114 us, with 256
-  // threads 131, with 1024 194); slices, which are short: 256
+  // rows that fill the GPU by themselves: 512 threads a row (2047 rows of 128256 at 1965 MHz: 114 us,
+  // with 256 threads 131, with 1024 194); slices, which are short: 256
   const int threads = splits > 1 ? lp::kSliceThreads : 512;
   auto kern = threads == 512 ? (bf16 ? lp::logprobs_kernel<true, 512> : lp::logprobs_kernel<false, 512>)
                              : (bf16 ? lp::logprobs_kernel<true, lp::kSliceThreads> : lp::logprobs_kernel<false, lp::kSliceThreads>);

@@ -40,7 +40,11 @@ class Decoder:
     """``layers``: DeviceLayer blocks of one rank and device; ``embedding`` fp32 [vocab, hidden];
     ``final_norm`` fp32 [hidden]; ``lm_head`` (weight bytes, type, vocab), a hidden x vocab
     matrix.  ``pages`` pages of ``page`` tokens hold the keys and values of every layer, up to
-    ``max_tokens`` a row."""
+    ``max_tokens`` a row.
+
+    Calls of more than DECODE_MAX_TOKENS rows in all (prompts) run their matmuls on bf16 inputs, and
+    their attention on bf16 queries with a bf16 result, so that it takes the tcgen05 kernel; up to as
+    many rows everything is fp32."""
 
     def __init__(self, layers: list[DeviceLayer], embedding: torch.Tensor, final_norm: torch.Tensor,
                  lm_head: tuple[torch.Tensor, object, int], pages: int, page: int = 64, max_tokens: int = 4096,
