@@ -15,10 +15,10 @@ from test_kv_gpu import DT, _check, _q
 pytestmark = pytest.mark.gpu
 
 
-def _two_scores(cuda, dtype, new, dim, values):
-    """8 KV heads of 8 query heads over 40960 tokens, of which the first 128 score 0 and the others
+def _two_scores(cuda, dtype, new, dim, values, L=40960):
+    """8 KV heads of 8 query heads over L tokens, of which the first 128 score 0 and the others
     7.8 log 2: (out, lse, the second score, codes, scales)."""
-    kv, group, page, L = 8, 8, 128, 40960
+    kv, group, page = 8, 8, 128
     n = L // page
     g = torch.Generator(device=cuda).manual_seed(dim)
     codes = torch.zeros((n, 1, 2, kv, page, dim), dtype=torch.int8, device=cuda)
@@ -87,3 +87,9 @@ def test_infinite_queries_give_nan_in_their_rows(cuda, dtype, new, value):
     out[0, :128] = torch.from_numpy(ref[0, 0]).to(out)
     lse[0, 0] = float(ref_lse[0, 0])
     _check(out, lse, ref, ref_lse, 127 * float(pool.scales.max()), dtype)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_half_a_million_equal_scores(cuda, dim):
+    """The sum's roundings do not grow with the cache."""
+    _two_scores(cuda, torch.bfloat16, 600, dim, True, L=524288)

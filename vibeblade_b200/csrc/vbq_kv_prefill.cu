@@ -513,7 +513,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
       // rows past the last hold zeros, are not written, and need no mask
       const int hi = live ? g.len - g.n + i : 0x3fffffff;
       const int lo = live && a.window > 0 ? hi - a.window + 1 : 0;
-      float mm = 0.0f, l = 0.0f;
+      float mm = 0.0f, l = 0.0f, rest = 0.0f;  // rest: what l's roundings left out
       bool seen = false;
       const int c0 = g.c0, c1 = g.c1, first = g.first;
       for (int j = c0; j < c1; ++j, ++count) {
@@ -556,6 +556,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
           const float f = move && seen ? ex2(-d) : 1.0f;
           mm += d;
           l *= f;
+          rest *= f;
           seen = seen || move;
           if (j > c0) {  // S of this run is there, so P V of the one before is done
 #pragma unroll 1
@@ -571,7 +572,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
             }
           }
         }
-        float of_run = 0.0f;  // added up by itself first: l takes a rounding a run, not one a block
+        float of_run = 0.0f;  // added up by itself first, as its roundings go one way where scores are equal
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           uint32_t pk[16];
@@ -598,7 +599,11 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
             if (lane == 0) mbar_arrive(smem_u32(&bars.p_half[half]));
           }
         }
-        l += of_run;
+        {  // l + rest, to l's own rounding and no more over any number of runs
+          const float add = of_run + rest, to_l = l + add;
+          rest = add - (to_l - l);
+          l = to_l;
+        }
         p_wait_st();
         p_fence_before();
         __syncwarp();
