@@ -23,7 +23,9 @@
 //
 // Rounding: codes and products are exact in fp16 and fp32; a query row is scaled by a power of
 // two into fp16's range, which keeps all of bf16's digits down to 2^-29 of its largest value (and
-// more coarsely 2^-39); weights are rounded to fp16's 11 bits, where the output keeps 8.
+// more coarsely 2^-39); weights are rounded to fp16's 11 bits, where the output keeps 8.  The sum of
+// exponentials is compensated; O is the tensor core's own fp32 sum, which truncates: rows of equal weights
+// come out 0.08 % low over 41000 tokens, 0.16 % over 524288, 0.37 % over a million (a bf16 step is 0.4 %).
 //
 // Measured (device time of a launch among others, 8 heads of 128): the last 2048 of 32768 tokens of 64
 // query heads, 2.13 TFLOP: 2.38 ms at 1627 MHz, where the power limit holds the SMs in a row of calls,
