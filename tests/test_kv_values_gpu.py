@@ -10,7 +10,7 @@ import torch
 
 import kv_reference as R
 import vibeblade_b200 as vb
-from test_kv_gpu import DT, _check, _q
+from test_kv_gpu import DT, _attend, _check, _q
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,12 @@ def test_infinite_queries_give_nan_in_their_rows(cuda, dtype, new, value):
 def test_half_a_million_equal_scores(cuda, dim):
     """The sum's roundings do not grow with the cache."""
     _two_scores(cuda, torch.bfloat16, 600, dim, True, L=524288)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 1 << 30])
+def test_the_largest_windows(cuda, dtype, dim, window):
+    """Beside rows before a sequence's first token, from whose places they would reach past int32."""
+    for lens, new in (([22, 0, 9, 3], [30, 12, 9, 10]), ([10, 40], [150, 170]), ([200], [230])):
+        _attend(cuda, lens, new, 8, 2, dim, 16, dtype, window=window, seed=dim)

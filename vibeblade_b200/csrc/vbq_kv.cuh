@@ -29,6 +29,12 @@ __device__ __forceinline__ int64_t block_index(const KvCache& c, int page, int w
   return (((int64_t)page * c.layers + c.layer) * 2 + which) * c.heads + head;
 }
 
+// The first key that a row whose last one is `hi` sees; what is before the sequence's first (hi < 0, where the
+// row sees nothing) is 0 too, so that no window reaches past int32.
+__device__ __forceinline__ int first_key(const KvAttention& a, int hi) {
+  return a.window > 0 && hi >= a.window ? hi - a.window + 1 : 0;
+}
+
 // A value block's scale as the attention's weights take it.  They carry it, and the sum of exponentials
 // takes its reciprocal: a block of zeros, whose scale is 0 and any would do, gets one that leaves the
 // sum of 2^24 tokens' weights (2^15 at most) in fp32 and lies below every scale that matters.

@@ -92,7 +92,7 @@ __device__ __forceinline__ Span span_of(const KvBatch& b, const KvAttention& a, 
   Span v;
   v.n = seq_new(b, s), v.len = seq_len(b, s);
   if ((int64_t)v.n * a.group > a.rows_upto) v.n = 0;  // another kernel's
-  v.lo = a.window > 0 ? max(0, v.len - v.n - a.window + 1) : 0;
+  v.lo = first_key(a, v.len - v.n);
   v.c0 = v.lo / kChunk;
   v.chunks = v.n > 0 ? max(1, (v.len + kChunk - 1) / kChunk - v.c0) : 0;
   v.tiles = (int)(((int64_t)v.n * a.group + tile_rows - 1) / tile_rows);
@@ -208,13 +208,12 @@ attn_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, int*
       for (int e = 0; e < 2; ++e) {
         const int i = (row_base + 8 * t + 2 * q4 + e) / a.group;
         hi[t][e] = i < v.n ? v.len - v.n + i : -1;
-        lo[t][e] = a.window > 0 ? hi[t][e] - a.window + 1 : 0;
+        lo[t][e] = first_key(a, hi[t][e]);
       }
     const int i0 = row_base / a.group, i1 = min(v.n - 1, (row_base + kRows - 1) / a.group);
     const int hi_min = v.len - v.n + i0;  // columns past the last row hold zeros and are never written
     const int hi_max = v.len - v.n + i1;
-    const int lo_min = a.window > 0 ? max(0, v.len - v.n + i0 - a.window + 1) : 0;
-    const int lo_max = a.window > 0 ? hi_max - a.window + 1 : 0;
+    const int lo_min = first_key(a, hi_min), lo_max = first_key(a, hi_max);
 
     // ---- blocks of 16 tokens: each warp a run of them ----
     const int first_tok = max((v.c0 + ch0) * kChunk, lo_min & ~(kBlockTokens - 1));

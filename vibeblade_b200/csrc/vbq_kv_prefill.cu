@@ -213,8 +213,7 @@ __device__ __forceinline__ PRun p_run(const PSeq& q, const KvAttention& a, int t
   const int i0 = (int)quotient((int64_t)tile * kTileRows, a.group);
   const int i1 = min(q.n - 1, (int)quotient((int64_t)tile * kTileRows + kTileRows - 1, a.group));
   const int hi = q.len - q.n + i1;
-  const int lo = a.window > 0 ? max(0, q.len - q.n + i0 - a.window + 1) : 0;
-  const int first = lo / kTok;
+  const int first = first_key(a, q.len - q.n + i0) / kTok;
   return {first, max(1, hi / kTok + 1 - first)};  // hi < 0: one run, all of it masked
 }
 // Runs of a sequence over all its tiles, and of its longest; the whole warp.
@@ -514,7 +513,7 @@ prefill_kernel(KvAttention a, KvCache c, KvBatch b, float* __restrict__ parts, i
 
       // rows past the last hold zeros, are not written, and need no mask
       const int hi = live ? g.len - g.n + i : 0x3fffffff;
-      const int lo = live && a.window > 0 ? hi - a.window + 1 : 0;
+      const int lo = live ? first_key(a, hi) : 0;
       float mm = 0.0f, l = 0.0f, rest = 0.0f;  // rest: what l's roundings left out
       bool seen = false;
       const int c0 = g.c0, c1 = g.c1, first = g.first;
